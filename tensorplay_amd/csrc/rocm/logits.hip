@@ -138,14 +138,16 @@ struct WaveScan {
 #pragma unroll
         for (int e = 1; e < N; ++e) cm = fmaxf(cm, v[e]);
         if (__any(cm > m)) {
-            const float top = wave_max_f(fmaxf(cm, m));
-            const float down = ex2((m - top) * k.k1);
-            r = fma(r, (double)(exact(k) * down), (double)(n * down));
-            n = 0.0f;
-            m = top;
+            // What is carried over becomes a term like those that follow, relative to the new
+            // mk and not to m: part() takes the rounding of mk out of all of them at once.
+            const float was = exact(k), d0 = m;
+            m = wave_max_f(fmaxf(cm, m));
             far = !(fabsf(m * k.k1) < kFar);
             base = far ? m : 0.0f;
             mk = far ? 0.0f : m * k.k1;
+            const float d = d0 - base, down = ex2(fmaf(d, k.k2, fmaf(d, k.k1, -mk)));
+            r = fma(r, (double)(was * down), (double)(n * down));
+            n = 0.0f;
             terms<N, true>(v, k);
         } else if (far) {
             terms<N, true>(v, k);
