@@ -828,13 +828,14 @@ __device__ __forceinline__ double pref_pair(const PrefArgs& a, long long i) {
     a.reward[i] = (float)rc;
     a.reward[i + a.pairs] = (float)rr;
     const double h = rc - rr;
-    // log(1 + e^h) and its derivative, without overflow
-    const double u = exp(-fabs(h)), soft = fmax(h, 0.0) + log1p(u);
-    const double up = (h >= 0.0 ? 1.0 : u) / (1.0 + u);
-    const double c = a.beta / (double)a.pairs * (up - (1.0 - a.eps));
+    // log(1 + e^-h) and log(1 + e^h), and their derivatives: each from e^-|h| without a
+    // difference, so that a pair far apart keeps the digits of its e^-|h|
+    const double u = exp(-fabs(h)), l = log1p(u);
+    const double up = (h >= 0.0 ? 1.0 : u) / (1.0 + u), down = (h >= 0.0 ? u : 1.0) / (1.0 + u);
+    const double c = a.beta / (double)a.pairs * (a.eps * up - (1.0 - a.eps) * down);
     a.sums[i] = c;
     a.sums[i + a.pairs] = -c;
-    return soft - (1.0 - a.eps) * h;
+    return (1.0 - a.eps) * (fmax(-h, 0.0) + l) + a.eps * (fmax(h, 0.0) + l);
 }
 __device__ __forceinline__ void pref_coef(const PrefArgs& a, long long q) {
     const Range r = range_of(a, q);
