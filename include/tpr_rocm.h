@@ -392,6 +392,8 @@ int tpr_policy_loss(const tpr_logits_desc* desc, const tpr_policy_desc* policy, 
  * i + pairs the other.  reward[i] = beta (sum logp - ref[i]), ref float32 [2 pairs];
  * with h = reward[i] - reward[i + pairs]:
  *   loss = 1/pairs sum -((1 - label_smoothing) log sigmoid(h) + label_smoothing log sigmoid(-h)).
+ * h is infinite where a token of one answer has logit -inf: a share of 0 then has no part
+ * of the loss, and NaN is left only where both answers have such a token.
  * coef[row] = dloss / dlogp, 0 for rows of no sequence. */
 size_t tpr_preference_loss_workspace_bytes(const tpr_logits_desc* desc, int64_t pairs);
 int tpr_preference_loss(const tpr_logits_desc* desc, int64_t pairs, double beta, double label_smoothing,

@@ -835,7 +835,9 @@ __device__ __forceinline__ double pref_pair(const PrefArgs& a, long long i) {
     const double c = a.beta / (double)a.pairs * (a.eps * up - (1.0 - a.eps) * down);
     a.sums[i] = c;
     a.sums[i + a.pairs] = -c;
-    return (1.0 - a.eps) * (fmax(-h, 0.0) + l) + a.eps * (fmax(h, 0.0) + l);
+    // h is infinite where a token of one answer has no probability: a share of 0 then has
+    // no part of the loss
+    return (a.eps < 1.0 ? (1.0 - a.eps) * (fmax(-h, 0.0) + l) : 0.0) + (a.eps > 0.0 ? a.eps * (fmax(h, 0.0) + l) : 0.0);
 }
 __device__ __forceinline__ void pref_coef(const PrefArgs& a, long long q) {
     const Range r = range_of(a, q);
