@@ -2,6 +2,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <numeric>
@@ -16,6 +17,16 @@ namespace {
 
 void hip_check(hipError_t e, const char* what) {
     if (e != hipSuccess) TP_THROW(RuntimeError, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+// Asked of the runtime until it says yes: host tensors never get here (the question starts
+// the HIP runtime, after which a process must not fork), and a device that was there stays.
+bool has_device(int index) {
+    static std::atomic<int> seen{0};
+    if (index < seen.load(std::memory_order_relaxed)) return true;
+    const int n = rocmDeviceCount();
+    seen.store(n, std::memory_order_relaxed);
+    return index < n;
 }
 
 int64_t wrap_dim(int64_t d, int64_t ndim, bool index_error) {
@@ -48,8 +59,7 @@ Tensor Tensor::empty(const std::vector<int64_t>& shape, DType dtype, const Devic
     auto st = std::make_shared<StorageImpl>();
     st->nbytes = (size_t)n * elementSize(dtype);
     st->device = device;
-    static const int devices = rocmDeviceCount();   // of this process, asked once
-    if (device.is_rocm() && device.index >= devices)
+    if (device.is_rocm() && !has_device(device.index))
         TP_THROW(RuntimeError, "ROCm device " + std::to_string(device.index) + " is not available");
     st->data = allocate(st->nbytes, device);
     auto impl = std::make_shared<TensorImpl>();
