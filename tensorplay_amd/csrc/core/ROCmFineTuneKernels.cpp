@@ -198,6 +198,8 @@ Block block(const Tensor& self, DType residual, const Tensor& pre_weight, double
         if (g->dim() == 0 || g->shape()[g->dim() - 1] != b.d.cols)
             TP_THROW(RuntimeError, std::string(op) + ": gate's last dim must be the input's");
         b.d.gates = b.d.cols ? g->numel() / b.d.cols : 0;
+        if (b.d.rows > 0 && b.d.gates == 0)   // the descriptor's "no gate"
+            TP_THROW(ValueError, std::string(op) + ": gates must divide the rows, and there are none");
         b.gate = arg(*g, self, self.dtype(), b.d.gates * b.d.cols, op, "gate");
     }
     return b;
