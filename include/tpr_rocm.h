@@ -419,7 +419,8 @@ int tpr_dropout(const void* in, int32_t dtype, int64_t rows, int64_t cols, doubl
  * the weights are of type dtype; h and out of residual_dtype: dtype or TPR_FLOAT32.
  * y is computed from out before its rounding.  rstd_post (NULL without a
  * post_weight) and rstd_pre, float32 [rows], are what the backward pass takes.
- * out may be h.  cols at most TPR_GATED_NORM_MAX_COLS. */
+ * out may be h.  cols at most TPR_GATED_NORM_MAX_COLS; without columns the roots are
+ * NaN, the mean of no squares, and are written where given. */
 #define TPR_GATED_NORM_MAX_COLS 16384
 typedef struct tpr_gated_norm_desc {
     int32_t dtype, residual_dtype;

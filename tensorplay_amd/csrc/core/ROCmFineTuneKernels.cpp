@@ -166,6 +166,13 @@ Tensor run_dropout(const Tensor& self, double p, int64_t seed, int64_t offset, c
     return out;
 }
 
+// Rows of a tensor, also where they have no columns
+int64_t leading(const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.shape()[i];
+    return n;
+}
+
 // What both passes of the end of a block share: descriptor and checked weights.
 struct Block {
     tpr_gated_norm_desc d;
@@ -184,7 +191,7 @@ Block block(const Tensor& self, DType residual, const Tensor& pre_weight, double
     Block b;
     std::memset(&b.d, 0, sizeof b.d);
     b.d.cols = self.shape()[self.dim() - 1];
-    b.d.rows = b.d.cols ? self.numel() / b.d.cols : 0;
+    b.d.rows = leading(self);
     b.d.dtype = (int32_t)self.dtype();
     b.d.residual_dtype = (int32_t)residual;
     b.d.eps = eps;
@@ -197,7 +204,7 @@ Block block(const Tensor& self, DType residual, const Tensor& pre_weight, double
     if (const Tensor* g = opt(gate)) {
         if (g->dim() == 0 || g->shape()[g->dim() - 1] != b.d.cols)
             TP_THROW(RuntimeError, std::string(op) + ": gate's last dim must be the input's");
-        b.d.gates = b.d.cols ? g->numel() / b.d.cols : 0;
+        b.d.gates = leading(*g);
         if (b.d.rows > 0 && b.d.gates == 0)   // the descriptor's "no gate"
             TP_THROW(ValueError, std::string(op) + ": gates must divide the rows, and there are none");
         b.gate = arg(*g, self, self.dtype(), b.d.gates * b.d.cols, op, "gate");

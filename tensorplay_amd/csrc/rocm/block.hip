@@ -284,6 +284,14 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_block_fwd(BlockArgs a) {
     }
 }
 
+// Rows of no columns: the mean of no squares is NaN, and so are the roots.
+__global__ __launch_bounds__(kBlk) void k_no_columns(float* rstd_post, float* rstd_pre, long long rows) {
+    const long long row = (long long)blockIdx.x * kBlk + threadIdx.x;
+    if (row >= rows) return;
+    if (rstd_post) rstd_post[row] = NAN;
+    if (rstd_pre) rstd_pre[row] = NAN;
+}
+
 struct BlockBwdArgs {
     BlockArgs b;
     const void *gy, *gout;
@@ -711,7 +719,13 @@ extern "C" int tpr_gated_norm(const tpr_gated_norm_desc* desc, const void* x, co
     DropArgs drop;
     const int rc = check_block(desc, who, drop);
     if (rc != TPR_OK) return rc;
-    if (desc->rows == 0 || desc->cols == 0) return TPR_OK;
+    if (desc->rows == 0) return TPR_OK;
+    if (desc->cols == 0) {
+        if (!rstd_post && !rstd_pre) return TPR_OK;
+        hipLaunchKernelGGL(k_no_columns, dim3((unsigned)((desc->rows + kBlk - 1) / kBlk)), dim3(kBlk), 0,
+                           static_cast<hipStream_t>(stream), rstd_post, rstd_pre, desc->rows);
+        return check_launch(who);
+    }
     if (!x || !h || !pre_weight || !out || !y || !rstd_pre || (post_weight && !rstd_post) || (desc->gates > 0 && !gate))
         return fail(TPR_ERR_INVALID_ARG, std::string(who) + ": null pointer");
     BlockArgs a = block_args(desc, drop);
