@@ -376,7 +376,9 @@ int tpr_token_logprob_backward(const tpr_logits_desc* desc, const float* coef, c
  * dloss / dlp, to be passed to tpr_token_logprob_backward with scale = the loss's
  * gradient; with grad not NULL the logits' gradient (of a loss gradient of 1) is
  * written here, and logp is all that is needed besides: lse and coef may then be
- * NULL. */
+ * NULL, and rows of up to 155648 logits in half precision, 77824 in float32, are read
+ * once.  A TPR_FLOAT16 gradient rounds what is below 2^-25 to 0: a loss scale goes through
+ * coef and `scale`. */
 typedef struct tpr_policy_desc {
     double clip_low, clip_high, kl_coef;
 } tpr_policy_desc;

@@ -62,7 +62,7 @@ struct DropoutArgs {
 // PASS: the stores pass the caches, in half precision from kDropoutPass bytes on: two
 // dropouts of [16384, 4096] bfloat16 one after the other 104 -> 89 us (6.0 TB/s), of
 // [8192, 4096] 43 -> 47.  float32 stores two halves of 32 bytes a thread, which must
-// meet in a cache: [16384, 4096] 95 -> 107 us.
+// meet in a cache: one dropout of [16384, 4096] 95 -> 107 us.
 constexpr long long kDropoutPass = 128LL << 20;
 
 template <class T, bool PASS>

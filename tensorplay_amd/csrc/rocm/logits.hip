@@ -8,10 +8,11 @@
 // backward pass reads the row once more and writes its gradient.
 //
 // Where one token is all but certain, s is 1 plus a rest that 32 bits would round
-// away, and logp is minus that rest: so the elements equal to the maximum are counted
-// (n) and only the others summed (r).  What is kept of a row is m and s - 1 =
-// n - 1 + r; log s = log1p(s - 1) has the rest's digits, and 1 - softmax at the target,
-// the gradient's largest element, is -expm1(logp).
+// away, and logp is minus that rest: so the element that sets the maximum is counted (n),
+// with the equal ones that arrive with it, and only the others summed (r).  Equal ones
+// that arrive later are summed, which costs no digits: s - 1 is then 1 and more.  What is
+// kept of a row is m and s - 1 = n - 1 + r; log s = log1p(s - 1) has the rest's digits, and
+// 1 - softmax at the target, the gradient's largest element, is -expm1(logp).
 //
 // Costs: a row is read once for its statistics (memory-bound from a few hundred rows on:
 // [4096, 151936] bfloat16 211 us, 5.9 TB/s; [2048, 50261] float16 38 us, 5.4 TB/s), read
@@ -41,8 +42,8 @@ namespace {
 constexpr int kLgBlock = 256;
 constexpr float kLowest = -3.40282347e38f;  // the first maximum: finite, so that x - m never is NaN for x = -inf
 
-// The state of a part of a row: maximum, how many elements equal it, and the sum of
-// exp((x - m) / T) over the others.  Nothing seen but -inf: n = r = 0.
+// The state of a part of a row: maximum, how many elements equal it of those that were
+// counted, and the sum of exp((x - m) / T) over the others.  Nothing seen but -inf: n = r = 0.
 struct RowPart {
     float m, n;
     double r;
@@ -107,7 +108,8 @@ struct WaveScan {
     bool far = true;                   // m k1 is past the range of the fused one
     double r = 0.0;
 
-    // TOP: some element may equal m, or m is far
+    // TOP: elements that equal m are counted: in the batch that has set m, and in every
+    // batch while m is far
     template <int N, bool TOP>
     __device__ __forceinline__ void terms(const float (&v)[N], const Scale& k) {
         float s[4] = {};
