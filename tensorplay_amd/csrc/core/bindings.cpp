@@ -137,7 +137,12 @@ struct TorchNames {
 
 // A torch tensor's memory as a Tensor: zero-copy on an AMD GPU, a copy on the host.
 Tensor from_torch(const py::object& o) {
-    static const auto* n = new TorchNames();
+    // The interpreter's lock orders this, and no lock of its own: a thread that waited for a
+    // guarded initialization would hold the lock that the import may have let go of.  Two
+    // threads may both look the names up; one set is kept.
+    static const TorchNames* names = nullptr;
+    if (!names) names = new TorchNames();
+    const TorchNames* const n = names;
     PyObject* t = o.ptr();
     if (steal(PyObject_GetAttr(t, n->is_cuda)).ptr() != Py_True)
         return from_numpy(py::array(o.attr("detach")().attr("numpy")()), std::nullopt, py::str("cpu"));
